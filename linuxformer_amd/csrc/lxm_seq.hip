@@ -331,21 +331,17 @@ __global__ __launch_bounds__(256) void gd_recurrent(lxm_seq_table S, lxm_gd_io i
 // T and A need no state: gd_prep forms them for all chunks at once. gd_run walks a sequence's chunks.
 //
 // Products on v_mfma_f32_16x16x32_bf16 (lane l: A[l % 16][8 (l / 16) + j], B[8 (l / 16) + j][l % 16],
-// D[4 (l / 16) + r][l % 16]) with float32's precision: a float32 is the sum of three bf16 (8 of its 24
-// significant bits each, cut off, nothing rounded), a float16 of two, and of a product of two such sums the terms
-// part i x part j with i + j <= 2 are taken: what is left out is below 2^-21 of it, 2^-24 on average. Keys and
-// queries go in as they were given (one part in bf16), their norms in the float32 factors beside the
-// products. One such product of bf16 by float32 takes 3 instructions of 16 cycles per 32 k where the float32
+// D[4 (l / 16) + r][l % 16]) with float32's precision, whatever the outputs' type: a float32 is the sum of three
+// bf16 (8 of its 24 significant bits each, cut off, nothing rounded), a float16 of two, and of a product of two such
+// sums the terms part i x part j with i + j <= 2 are taken: what is left out is below 2^-21 of it, 2^-24 on
+// average. Keys and queries go in as they were given (one part in bf16), their norms in the float32 factors
+// beside the products. One such product of bf16 by float32 takes 3 instructions of 16 cycles per 32 k where the float32
 // instruction takes 8 of 32.
 //
 // 2,048 positions of 32 heads, bf16, 128 x 128: 60 to 68 us (gd_prep 17, gd_run 51), where the fp32 matrix
 // instructions and a workspace of 75 KB a (head, chunk) take 234 for the same sums of float32 inputs.
 template <int TY>
 constexpr int kParts = TY == LXM_BF16 ? 1 : TY == LXM_FP16 ? 2 : 3;
-// The parts of A, D and the state in the products that only the output sees: a bf16 output is rounded at 2^-9; two
-// parts of each leave at most 2^-13 of a product, the smaller times the smaller among it.
-template <int TY>
-constexpr int kOut = TY == LXM_BF16 ? 2 : 3;
 
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
@@ -392,8 +388,7 @@ __device__ __forceinline__ f32x4 product(const u32x4* a, const u32x4* b, f32x4 c
 constexpr int kFrag = 1024;
 template <int TY, int K>
 constexpr int kKeyWs = 3 * (64 * K * 2) * kParts<TY>;
-template <int TY>
-constexpr int kHeadWs = 6 * (3 + kOut<TY>)*kFrag + 5 * 256;
+constexpr int kHeadWs = 6 * (3 + 3) * kFrag + 5 * 256;
 
 __device__ __forceinline__ int block_of(int tile, int p) { return tile < 2 ? tile : 2 * tile - 2 + p; }  // 0, 1, 2 3, 4 5
 
@@ -499,7 +494,7 @@ __device__ __forceinline__ void invert(float* l, int lane) {
 template <int TY, int K>
 __global__ __launch_bounds__(256) void gd_prep(lxm_seq_table S, lxm_gd_io io, char* ws, int c0) {
   typedef typename Elem<TY>::T T;
-  constexpr int NP = kParts<TY>, NO = kOut<TY>, NB = K / 32, RS = K + 8;
+  constexpr int NP = kParts<TY>, NB = K / 32, RS = K + 8;
   extern __shared__ __align__(16) char lds[];
   PrepLds& m = *(PrepLds*)lds;
   uint16_t* kt = (uint16_t*)(lds + sizeof(PrepLds));
@@ -511,7 +506,7 @@ __global__ __launch_bounds__(256) void gd_prep(lxm_seq_table S, lxm_gd_io io, ch
   const int lane = threadIdx.x & 63, wave = wave_of(), g = lane >> 4, c = lane & 15, row = wave * 16 + c;
   const int nv = io.nk * io.r;
   char* wk = ws + ((int64_t)ci * io.nk + kh) * kKeyWs<TY, K>;
-  char* wh = ws + (int64_t)(gridDim.x / groups) * kKeyWs<TY, K> + ((int64_t)ci * nv + kh * io.r + h0) * kHeadWs<TY>;
+  char* wh = ws + (int64_t)(gridDim.x / groups) * kKeyWs<TY, K> + ((int64_t)ci * nv + kh * io.r + h0) * kHeadWs;
 
   // the wave's 16 rows, dims 32 i + 8 g .. + 7
   u32x4 kf[NB][NP], qf[NB][NP];
@@ -612,7 +607,7 @@ __global__ __launch_bounds__(256) void gd_prep(lxm_seq_table S, lxm_gd_io io, ch
     const double last = __shfl(gc, 63);  // (positions past n add nothing)
     m.gc[wave][lane] = gc;
     m.beta[wave][lane] = be;
-    float* fac = (float*)(wh + wave * (int64_t)kHeadWs<TY> + 6 * (3 + NO) * kFrag);
+    float* fac = (float*)(wh + wave * (int64_t)kHeadWs + 6 * (3 + 3) * kFrag);
     const float e = __builtin_amdgcn_exp2f((float)gc), kr = m.rk[lane];
     fac[lane] = be;
     fac[64 + lane] = be * e * kr;
@@ -625,7 +620,7 @@ __global__ __launch_bounds__(256) void gd_prep(lxm_seq_table S, lxm_gd_io io, ch
     float* l = mat + h * (64 * kLd);
     const double gi = m.gc[h][row];
     const float bi = m.beta[h][row] * rk;
-    char* to = wh + h * (int64_t)kHeadWs<TY> + 6 * 3 * kFrag + lane * 16;
+    char* to = wh + h * (int64_t)kHeadWs + 6 * 3 * kFrag + lane * 16;
     double gk[2][8];
     float rkey[2][8];
 #pragma unroll
@@ -647,10 +642,10 @@ __global__ __launch_bounds__(256) void gd_prep(lxm_seq_table S, lxm_gd_io io, ch
       }
       *(f32x4*)&l[row * kLd + 32 * p + 8 * g] = lo[0];
       *(f32x4*)&l[row * kLd + 32 * p + 8 * g + 4] = lo[1];
-      u32x4 f[NO];
-      parts<8, NO>(x, (uint32_t(*)[4])f);
+      u32x4 f[3];
+      parts<8, 3>(x, (uint32_t(*)[4])f);
 #pragma unroll
-      for (int s = 0; s < NO; s++) *(u32x4*)(to + (block_of(wave, p) * NO + s) * kFrag) = f[s];
+      for (int s = 0; s < 3; s++) *(u32x4*)(to + (block_of(wave, p) * 3 + s) * kFrag) = f[s];
     }
   }
   __syncthreads();
@@ -658,7 +653,7 @@ __global__ __launch_bounds__(256) void gd_prep(lxm_seq_table S, lxm_gd_io io, ch
   __syncthreads();
   for (int u = wave; u < 6 * nh; u += 4) {
     const int h = u / 6, e = u % 6, tile = e < 2 ? e : (e + 2) / 2, p = e < 2 ? 0 : e & 1;
-    char* to = wh + h * (int64_t)kHeadWs<TY> + lane * 16;
+    char* to = wh + h * (int64_t)kHeadWs + lane * 16;
     const f32x4* src = (const f32x4*)(mat + h * (64 * kLd) + (tile * 16 + c) * kLd + 32 * p + 8 * g);
     const f32x4 x0 = src[0], x1 = src[1];
     float x[8];
@@ -682,9 +677,9 @@ __global__ __launch_bounds__(256) void gd_prep(lxm_seq_table S, lxm_gd_io io, ch
 template <int TY, int K, int NC>
 struct Run {
   typedef typename Elem<TY>::T T;
-  static constexpr int NP = kParts<TY>, NO = kOut<TY>, NB = K / 32, NT = K < 128 ? 1 : K / 128;
+  static constexpr int NP = kParts<TY>, NB = K / 32, NT = K < 128 ? 1 : K / 128;
   struct Lds {
-    u32x4 s[NC][NB][3][64], r[NC][2][3][64], d[NC][2][NO][64], e[NC][2][3][64];
+    u32x4 s[NC][NB][3][64], r[NC][2][3][64], d[NC][2][3][64], e[NC][2][3][64];
   };
   const lxm_gd_io& io;
   Lds& m;
@@ -696,15 +691,14 @@ struct Run {
   float eg;
 
   __device__ u32x4 frag(const char* base, int i) const { return *(const u32x4*)(base + i * kFrag + (uint32_t)(lane * 16)); }
-  __device__ const char* factors() const { return wh + 6 * (3 + NO) * kFrag; }
+  __device__ const char* factors() const { return wh + 6 * (3 + 3) * kFrag; }
   // a D tile (rows 4 g + r of tile t) as part of a right operand of blocks of 32 rows
-  template <int N>
   __device__ void put(u32x4 (*d)[64], f32x4 v, int t) const {
-    uint32_t p[N][2];
+    uint32_t p[3][2];
     float y[4] = {v[0], v[1], v[2], v[3]};
-    parts<4, N>(y, p);
+    parts<4, 3>(y, p);
 #pragma unroll
-    for (int i = 0; i < N; i++)
+    for (int i = 0; i < 3; i++)
       *(u32x2*)((char*)&d[i][c + 16 * (2 * (t & 1) + g / 2)] + 8 * (g & 1)) = u32x2{p[i][0], p[i][1]};
   }
   __device__ void put_state() const {
@@ -712,7 +706,7 @@ struct Run {
 #pragma unroll
       for (int n = 0; n < NC; n++)
 #pragma unroll
-        for (int t = 0; t < NT; t++) put<3>(m.s[n][(tile0 + t) / 2], s[n][t], tile0 + t);
+        for (int t = 0; t < NT; t++) put(m.s[n][(tile0 + t) / 2], s[n][t], tile0 + t);
     }
   }
   // one row tile of a left operand over the K dims
@@ -723,13 +717,12 @@ struct Run {
       for (int e = 0; e < NP; e++) f[i][e] = frag(base, (w * NB + i) * NP + e);
   }
   // one row tile of a triangular left operand (row tiles 0 and 1 have no second block: it stays zero)
-  template <int N>
-  __device__ void load_tri(u32x4 (*f)[N], const char* base) const {
+  __device__ void load_tri(u32x4 (*f)[3], const char* base) const {
 #pragma unroll
     for (int p = 0; p < 2; p++)
       if (p == 0 || w >= 2) {
 #pragma unroll
-        for (int e = 0; e < N; e++) f[p][e] = frag(base, block_of(w, p) * N + e);
+        for (int e = 0; e < 3; e++) f[p][e] = frag(base, block_of(w, p) * 3 + e);
       }
   }
   __device__ void load_x() {
@@ -742,12 +735,11 @@ struct Run {
     eg = ((const float*)factors())[256];
   }
   __device__ f32x4 factor(int i) const { return *(const f32x4*)(factors() + 256 * i + 64 * w + (uint32_t)(16 * g)); }
-  template <int N>
-  __device__ void operand(u32x4 (*f)[N], const u32x4 (*from)[N][64]) const {  // a right operand's two blocks
+  __device__ void operand(u32x4 (*f)[3], const u32x4 (*from)[3][64]) const {  // a right operand's two blocks
 #pragma unroll
     for (int p = 0; p < 2; p++)
 #pragma unroll
-      for (int e = 0; e < N; e++) f[p][e] = from[p][e][lane];
+      for (int e = 0; e < 3; e++) f[p][e] = from[p][e][lane];
     issued();
   }
   // S <- decay S + sum_i k_i e_i^T; then (wk, wh: the next chunk's) what the next needs for it
@@ -755,7 +747,7 @@ struct Run {
 #pragma unroll
     for (int n = 0; n < NC; n++) {
       u32x4 ef[2][3];
-      operand<3>(ef, m.e[n]);
+      operand(ef, m.e[n]);
 #pragma unroll
       for (int t = 0; t < NT; t++) s[n][t] *= eg;
 #pragma unroll
@@ -766,17 +758,20 @@ struct Run {
     put_state();
     load_x();
   }
-  template <int N>
+  template <int AT>  // blocks of the state in registers at a time
   __device__ f32x4 times_state(const u32x4 (*f)[NP], int n) const {
     f32x4 a[2] = {};
-    u32x4 sf[NB][N];
 #pragma unroll
-    for (int i = 0; i < NB; i++)
+    for (int i0 = 0; i0 < NB; i0 += AT) {
+      u32x4 sf[AT][3];
 #pragma unroll
-      for (int e = 0; e < N; e++) sf[i][e] = m.s[n][i][e][lane];
-    issued();
+      for (int i = 0; i < AT; i++)
 #pragma unroll
-    for (int i = 0; i < NB; i++) a[i & 1] = product<NP, N, N - 1>(f[i], sf[i], a[i & 1]);
+        for (int e = 0; e < 3; e++) sf[i][e] = m.s[n][i0 + i][e][lane];
+      issued();
+#pragma unroll
+      for (int i = 0; i < AT; i++) a[i & 1] = product<NP, 3, 2>(f[i0 + i], sf[i], a[i & 1]);
+    }
     return a[0] + a[1];
   }
 
@@ -814,14 +809,14 @@ struct Run {
       lds_barrier();
       f32x4 ks[NC];
 #pragma unroll
-      for (int n = 0; n < NC; n++) ks[n] = times_state<3>(kf, n);
+      for (int n = 0; n < NC; n++) ks[n] = times_state<NB>(kf, n);
       load_rows(kf, wk + 64 * K * 2 * NP);
 #pragma unroll
       for (int n = 0; n < NC; n++) {
         f32x4 R;
 #pragma unroll
         for (int r = 0; r < 4; r++) R[r] = fma(-ck[r], ks[n][r], be[r] * up<TY>(v[n][r]));
-        put<3>(m.r[n][w / 2], R, w);
+        put(m.r[n][w / 2], R, w);
       }
       if (more) t0 += LXM_SEQ_CHUNK, vp += LXM_SEQ_CHUNK * ts;
       load_v();
@@ -829,13 +824,13 @@ struct Run {
 #pragma unroll
       for (int n = 0; n < NC; n++) {
         u32x4 rf[2][3];
-        operand<3>(rf, m.r[n]);
+        operand(rf, m.r[n]);
         f32x4 d = {0, 0, 0, 0}, d1 = {0, 0, 0, 0};
         d = product<3, 3, 2>(tf[0], rf[0], d);
         d1 = product<3, 3, 2>(tf[1], rf[1], d1);
         d += d1;
-        put<3>(m.e[n][w / 2], d * cd, w);
-        put<NO>(m.d[n][w / 2], d, w);
+        put(m.e[n][w / 2], d * cd, w);
+        put(m.d[n][w / 2], d, w);
       }
       load_tri(tf, wh), cd = factor(3);
       lds_barrier();
@@ -846,7 +841,7 @@ struct Run {
 
   // waves 4 to 7
   __device__ void output(int chunks, int64_t kstep, int64_t hstep, int t0, int end, T* op) {
-    u32x4 qf[NB][NP], af[2][NO] = {};
+    u32x4 qf[NB][NP], af[2][3] = {};
     f32x4 cq, o[NC] = {};
     const int64_t ts = io.o_ts;
     const int row = w * 16 + 4 * g;
@@ -854,10 +849,10 @@ struct Run {
     auto finish = [&] {  // o of the chunk before
 #pragma unroll
       for (int n = 0; n < NC; n++) {
-        u32x4 df[2][NO];
-        operand<NO>(df, m.d[n]);
+        u32x4 df[2][3];
+        operand(df, m.d[n]);
 #pragma unroll
-        for (int p = 0; p < 2; p++) o[n] = product<NO, NO, NO - 1>(af[p], df[p], o[n]);
+        for (int p = 0; p < 2; p++) o[n] = product<3, 3, 2>(af[p], df[p], o[n]);
         if (t0 + LXM_SEQ_CHUNK <= end) {
 #pragma unroll
           for (int r = 0; r < 4; r++) op[r * ts + 16 * n] = down<TY>(o[n][r]);
@@ -881,7 +876,7 @@ struct Run {
       }
       lds_barrier();
 #pragma unroll
-      for (int n = 0; n < NC; n++) o[n] = times_state<NO>(qf, n) * cq;
+      for (int n = 0; n < NC; n++) o[n] = times_state<NB / 2>(qf, n) * cq;
       load_rows(qf, wk), cq = factor(2);
       lds_barrier();
       step_state();
@@ -891,8 +886,10 @@ struct Run {
   }
 };
 
+// (Four waves a SIMD where the registers allow it, two workgroups a CU: 24 ragged prompts of bf16 118 us with 4
+// registers spilled, 139 with 136 registers and one workgroup.)
 template <int TY, int K, int NC>
-__global__ __launch_bounds__(512) void gd_run(lxm_seq_table S, lxm_gd_io io, const char* ws, int c0, int n_chunks,
+__global__ __launch_bounds__(512, TY == LXM_BF16 && K <= 128 ? 4 : 2) void gd_run(lxm_seq_table S, lxm_gd_io io, const char* ws, int c0, int n_chunks,
                                               const float* carry, float* carry_to) {
   typedef typename Elem<TY>::T T;
   typedef Run<TY, K, NC> R;
@@ -908,10 +905,10 @@ __global__ __launch_bounds__(512) void gd_run(lxm_seq_table S, lxm_gd_io io, con
   if (a0 >= a1) return;
   const int lane = threadIdx.x & 63, wave = wave_of(), g = lane >> 4, c = lane & 15, w = wave & 3;
 
-  const int64_t kstep = (int64_t)io.nk * kKeyWs<TY, K>, hstep = (int64_t)nv * kHeadWs<TY>;
+  const int64_t kstep = (int64_t)io.nk * kKeyWs<TY, K>, hstep = (int64_t)nv * kHeadWs;
   R run{io, lds, lane, w, g, c, K < 128 ? w : wave * R::NT, K >= 128 || wave < 4,
         ws + (h / io.r) * (int64_t)kKeyWs<TY, K> + (a0 - c0) * kstep,
-        ws + n_chunks * kstep + (a0 - c0) * hstep + h * (int64_t)kHeadWs<TY>};
+        ws + n_chunks * kstep + (a0 - c0) * hstep + h * (int64_t)kHeadWs};
   const bool from = slot >= 0 || a0 > f0, to = slot >= 0 || a1 < f1;
   const int col = cb * 16 * NC + c;
   // (a sequence without a slot that goes on in another group of chunks: from the last launch's carry to the next's, of
@@ -981,7 +978,7 @@ constexpr int64_t kTwo = 600;
 template <int TY, int K>
 int chunks(const lxm_seq_table* s, const lxm_gd_io* io, char* ws, int64_t ws_bytes, hipStream_t st) {
   const int nv = io->nk * io->r, per = (nv + 7) / 8;
-  const int64_t carry = 2 * (int64_t)nv * K * io->V * 4, each = (int64_t)io->nk * kKeyWs<TY, K> + (int64_t)nv * kHeadWs<TY>;
+  const int64_t carry = 2 * (int64_t)nv * K * io->V * 4, each = (int64_t)io->nk * kKeyWs<TY, K> + (int64_t)nv * kHeadWs;
   if (ws_bytes < carry + each) return hipErrorInvalidValue;
   int64_t group = (ws_bytes - carry) / each;
   if (group > s->n_chunks) group = s->n_chunks;
@@ -1041,7 +1038,7 @@ template <int TY>
 int64_t ws_of(const lxm_gd_io* io, int64_t n) {
   const int64_t nv = (int64_t)io->nk * io->r;
   const int64_t key = io->K == 64 ? kKeyWs<TY, 64> : io->K == 128 ? kKeyWs<TY, 128> : kKeyWs<TY, 256>;
-  return 2 * nv * io->K * io->V * 4 + n * (io->nk * key + nv * kHeadWs<TY>);
+  return 2 * nv * io->K * io->V * 4 + n * (io->nk * key + nv * kHeadWs);
 }
 
 }  // namespace
