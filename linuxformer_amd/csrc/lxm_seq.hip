@@ -332,10 +332,12 @@ __global__ __launch_bounds__(256) void gd_recurrent(lxm_seq_table S, lxm_gd_io i
 //
 // Products on v_mfma_f32_16x16x32_bf16 (lane l: A[l % 16][8 (l / 16) + j], B[8 (l / 16) + j][l % 16],
 // D[4 (l / 16) + r][l % 16]) with float32's precision, whatever the outputs' type: a float32 is the sum of three
-// bf16 (8 of its 24 significant bits each, cut off, nothing rounded), a float16 of two, and of a product of two such
-// sums the terms part i x part j with i + j <= 2 are taken: what is left out is below 2^-21 of it, 2^-24 on
-// average. Keys and queries go in as they were given (one part in bf16), their norms in the float32 factors
-// beside the products. One such product of bf16 by float32 takes 3 instructions of 16 cycles per 32 k where the float32
+// bf16 (8 of its 24 significant bits each, cut off, nothing rounded), a float16 of two, and a product of two such
+// sums the sum of their parts' products but for the third by the third, below 2^-30 of it. (Without the second by
+// the third, too, up to 2^-21 would be lost, always towards zero, for 231 us against 239 of 24 ragged prompts in
+// fp32; parts rounded to nearest would lose 2^-23, but take longer to form: a bf16 prompt 72.9 us against 65.6.)
+// Keys and queries go in as they were given (one part in bf16), their norms in the float32 factors beside the
+// products. One such product of bf16 by float32 takes 3 instructions of 16 cycles per 32 k where the float32
 // instruction takes 8 of 32.
 //
 // 2,048 positions of 32 heads, bf16, 128 x 128: 60 to 68 us (gd_prep 17, gd_run 51), where the fp32 matrix
@@ -370,11 +372,11 @@ __device__ __forceinline__ void parts(const float* x, uint32_t (*p)[N / 2]) {
 // loads before this are requested before anything after it
 __device__ __forceinline__ void issued() { asm volatile("" ::: "memory"); }
 
-// acc += A B over one block of 32 k: the parts' products, small ones first
-template <int NA, int NB, int MAX>
+// acc += A B over one block of 32 k: the parts' products, small ones first, without the last by the last of three
+template <int NA, int NB>
 __device__ __forceinline__ f32x4 product(const u32x4* a, const u32x4* b, f32x4 c) {
 #pragma unroll
-  for (int sum = MAX; sum >= 0; sum--)
+  for (int sum = NA + NB < 6 ? NA + NB - 2 : 3; sum >= 0; sum--)
 #pragma unroll
     for (int i = 0; i < NA; i++)
       if (sum - i >= 0 && sum - i < NB) c = mfma(a[i], b[sum - i], c);
@@ -578,8 +580,8 @@ __global__ __launch_bounds__(256) void gd_prep(lxm_seq_table S, lxm_gd_io io, ch
           u32x4 f[NP];
 #pragma unroll
           for (int s = 0; s < NP; s++) f[s] = *(const u32x4*)&kt[(s * 64 + key) * RS + 32 * i + 8 * g];
-          x = product<NP, NP, 2>(f, kf[i], x);
-          y = product<NP, NP, 2>(f, qf[i], y);
+          x = product<NP, NP>(f, kf[i], x);
+          y = product<NP, NP>(f, qf[i], y);
         }
         settle(x);
         settle(y);
@@ -753,7 +755,7 @@ struct Run {
 #pragma unroll
       for (int p = 0; p < 2; p++)
 #pragma unroll
-        for (int t = 0; t < NT; t++) s[n][t] = product<NP, 3, 2>(xf[t][p], ef[p], s[n][t]);
+        for (int t = 0; t < NT; t++) s[n][t] = product<NP, 3>(xf[t][p], ef[p], s[n][t]);
     }
     put_state();
     load_x();
@@ -770,7 +772,7 @@ struct Run {
         for (int e = 0; e < 3; e++) sf[i][e] = m.s[n][i0 + i][e][lane];
       issued();
 #pragma unroll
-      for (int i = 0; i < AT; i++) a[i & 1] = product<NP, 3, 2>(f[i0 + i], sf[i], a[i & 1]);
+      for (int i = 0; i < AT; i++) a[i & 1] = product<NP, 3>(f[i0 + i], sf[i], a[i & 1]);
     }
     return a[0] + a[1];
   }
@@ -826,8 +828,8 @@ struct Run {
         u32x4 rf[2][3];
         operand(rf, m.r[n]);
         f32x4 d = {0, 0, 0, 0}, d1 = {0, 0, 0, 0};
-        d = product<3, 3, 2>(tf[0], rf[0], d);
-        d1 = product<3, 3, 2>(tf[1], rf[1], d1);
+        d = product<3, 3>(tf[0], rf[0], d);
+        d1 = product<3, 3>(tf[1], rf[1], d1);
         d += d1;
         put(m.e[n][w / 2], d * cd, w);
         put(m.d[n][w / 2], d, w);
@@ -852,7 +854,7 @@ struct Run {
         u32x4 df[2][3];
         operand(df, m.d[n]);
 #pragma unroll
-        for (int p = 0; p < 2; p++) o[n] = product<3, 3, 2>(af[p], df[p], o[n]);
+        for (int p = 0; p < 2; p++) o[n] = product<3, 3>(af[p], df[p], o[n]);
         if (t0 + LXM_SEQ_CHUNK <= end) {
 #pragma unroll
           for (int r = 0; r < 4; r++) op[r * ts + 16 * n] = down<TY>(o[n][r]);
