@@ -4,7 +4,9 @@
 // With m a row's maximum, s = sum exp(x - m) and w = sum exp(x - m) (x - m):
 //   lse = m + log s,  logprob = (x_t - m) - log s,  entropy = log s - w / s
 // (w rather than sum p x: no large numbers cancel). A thread keeps its own m, s and w, moved to a new maximum
-// once per kEach elements: s' = f s, w' = f (w + s (m - m')), f = exp(m - m').
+// once per kEach elements: s' = f s, w' = f (w + s (m - m')), f = exp(m - m'). A block's kEach terms are summed by
+// themselves and then added to s and w with what that rounds off kept beside them: a row's sums are as good as a
+// block's, however long it is and where equal terms round the same way each time.
 //
 // The alternatives: a wave walks its part of the row in blocks of 64 x kEach elements with a list of the best in LDS,
 // and no barrier. Where a block has more of use than `top`, a bound that `top` lanes' maxima reach cuts it first.
@@ -160,6 +162,12 @@ __device__ __forceinline__ void move(float& s, float& w, float d) {
   w = f * __builtin_fmaf(s, d, w);
   s *= f;
 }
+// s += x, what the addition rounds off added to l
+__device__ __forceinline__ void add_up(float& s, float& l, float x) {
+  const float t = s + x;
+  l += x - (t - s);
+  s = t;
+}
 // a wave's sums and maximum, in every lane (DPP: row shifts within 16 lanes, then the rows' last lanes)
 template <int CTRL, int ROWS, class T>
 __device__ __forceinline__ T dpp(T x, T rest) {
@@ -223,9 +231,10 @@ struct Part {
 
 // One workgroup per (row, part). Between the row's first and last 16-byte boundary a part is whole words, dealt to the
 // waves 64 at a time, kEach elements a lane of a block; what the row has before and after (less than a word each) is
-// a block of one element a lane, before the first and after the last of the row.
+// a block of one element a lane, before the first and after the last of the row. (Waves a SIMD: 2,048 bf16 rows of
+// 248,320 in 210 us with 5, 216 with 4; fp32 would spill 32 registers with 5, 1,200 rows of 150,001 in 223 us for 164.)
 template <int TY, int kEach>
-__global__ __launch_bounds__(kThreads) void score_part(lxm_score_io io, int n_parts, int words_per_part, Part* parts, double* lists) {
+__global__ __launch_bounds__(kThreads, TY == 2 ? 4 : 5) void score_part(lxm_score_io io, int n_parts, int words_per_part, Part* parts, double* lists) {
   typedef typename Elem<TY>::T T;
   constexpr int kVec = 16 / sizeof(T), U = kEach / kVec, kStep = kThreads * U;
   constexpr uint32_t kAll = kEach == 32 ? 0xffffffffu : (1u << kEach % 32) - 1;
@@ -253,6 +262,7 @@ __global__ __launch_bounds__(kThreads) void score_part(lxm_score_io io, int n_pa
   else if (xt == xt && xt != -kInf) below = __uint_as_float(__float_as_uint(xt) + (xt > 0 ? -1 : 1));
 
   float m = -kInf, s = 0, w = 0, gate = -kInf;
+  float ls = 0, lw = 0;  // what the additions to s and w have rounded off
   int c = 0, n = 0;
   double* list = l.list[wave];
   // -1: the elements before the words; -2: those behind
@@ -293,24 +303,28 @@ __global__ __launch_bounds__(kThreads) void score_part(lxm_score_io io, int n_pa
 #pragma unroll
     for (int i = 1; i < kEach; i++) hi = fmaxf(hi, v[i]), lo = fminf(lo, v[i]);
     if (hi > m) {
+      s += ls, w += lw, ls = lw = 0;
       move(s, w, m - hi);
       m = hi;
     }
+    float bs = 0, bw = 0;  // the block's
     if (lo - m > -200.f) {
 #pragma unroll
       for (int i = 0; i < kEach; i++) {
         const float y = v[i] - m, e = __builtin_amdgcn_exp2f(y * kLog2e);
-        s += e;
-        w = __builtin_fmaf(e, y, w);
+        bs += e;
+        bw = __builtin_fmaf(e, y, bw);
       }
     } else {  // (exp is 0 there; 0 x -inf is not, and NaN stays NaN)
 #pragma unroll
       for (int i = 0; i < kEach; i++) {
         const float d = v[i] - m, y = d < -200.f || v[i] == -kInf ? -200.f : d, e = __builtin_amdgcn_exp2f(y * kLog2e);
-        s += e;
-        w = __builtin_fmaf(e, y, w);
+        bs += e;
+        bw = __builtin_fmaf(e, y, bw);
       }
     }
+    add_up(s, ls, bs);
+    add_up(w, lw, bw);
     const bool odd = s != s;  // (a NaN or +inf was met: maxima say nothing)
     if (xt == xt && __any(!(hi < xt) || odd)) {
 #pragma unroll
@@ -375,6 +389,7 @@ __global__ __launch_bounds__(kThreads) void score_part(lxm_score_io io, int n_pa
     j = j == -1 ? (j0 < j1 ? j0 : -2) : j + kStep < j1 ? j + kStep : -2;
     if (j == -2 && (part != n_parts - 1 || tail == V)) break;
   }
+  s += ls, w += lw;
   // the token's own word was compared with xt: its lower tokens' equals count too
   const bool word = t >= head && t < tail;
   const int ts = word ? head + ((int)t - head) / kVec * kVec : (int)t;  // (its first token)

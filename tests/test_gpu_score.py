@@ -149,3 +149,22 @@ def test_top_is_read_at_each_call(cuda):
     assert token_logprobs(x, t, top=top).top_tokens.shape == (3, 2)
     top.fill_(5)
     assert token_logprobs(x, t, top=top).top_tokens.shape == (3, 5)
+
+
+def test_long_sums_of_equal_terms(cuda):
+    """Rows of one value behind the maximum, whose equal terms round the same way at each addition, in rows of one
+    part. Steps of 2^-24 of the sum: a term is within 3.25 (its argument's product and constant at |x - m| <= 1: 1.25;
+    exp2: 2), 32 equal terms added one after another within 16.5, their sums, joined without loss, 2, 10 joins of waves
+    and lanes: 32 of s. The log moves by as much and rounds by 16 (a step at 12.5), the last difference by 8: 56,
+    below 2^-18. w / s is at most 1 and has both sums' errors and 2 roundings, w's terms one more: 70 beside the log's
+    48, below 2^-17."""
+    print("[gpu-test] score, long sums", flush=True)
+    c = torch.arange(1, 17) / 16
+    x = torch.zeros(1024, 248320, dtype=BF, device=cuda)
+    x[:, 8320:] = -c.repeat(64)[:, None].to(cuda)  # (every thread of 32 elements in turn has met the maximum)
+    r = token_logprobs(x, torch.zeros(1024, dtype=torch.int32, device=cuda))
+    n, c = 240000, c.double()
+    s = 8320 + n * torch.exp(-c)
+    ref, entropy = -s.log(), s.log() + n * c * torch.exp(-c) / s
+    assert (r.logprob.double().cpu() - ref.repeat(64)).abs().max() <= 2.0 ** -18
+    assert (r.entropy.double().cpu() - entropy.repeat(64)).abs().max() <= 2.0 ** -17
