@@ -61,24 +61,17 @@ def token_logprobs(logits, tokens, top=0):
         return token_logprobs(logits.contiguous(), tokens.contiguous(), top)
     io, need = call
     N, k = io.rows, io.top
+    # (tensors of their own: a caller may change one in place, keep or save it without the others)
+    f32, i32 = torch.float32, torch.int32
+    out = Scores(logits.new_empty(N, dtype=f32), logits.new_empty(N, dtype=f32), logits.new_empty(N, dtype=i32),
+                 logits.new_empty((N, k), dtype=i32), logits.new_empty((N, k), dtype=f32))
     if N == 0:
-        return Scores(*(logits.new_empty(n, dtype=d) for n, d in (
-            (0, torch.float32), (0, torch.float32), (0, torch.int32), ((0, k), torch.int32),
-            ((0, k), torch.float32))))
-    # one allocation: the results and, behind them, the call's workspace
-    f = logits.new_empty(3 * N + 2 * N * k + need // 4 + 4, dtype=torch.float32)
-    logprob, entropy, top_logprobs, whole, _ = f.split_with_sizes((N, N, N * k, N + N * k, need // 4 + 4))
-    rank, top_tokens = whole.view(torch.int32).split_with_sizes((N, N * k))
-    out = Scores(logprob, entropy, rank, top_tokens.view(N, k), top_logprobs.view(N, k))
+        return out
+    ws = logits.new_empty(need, dtype=torch.uint8) if need else None
     io = ScoreIO.from_buffer_copy(io)
     io.logits, io.tokens = logits.data_ptr(), tokens.data_ptr()
-    io.logprob = p = f.data_ptr()
-    io.entropy = p + 4 * N
-    io.top_logprobs = p + 8 * N
-    io.rank = p + 8 * N + 4 * N * k
-    io.top_tokens = p + 12 * N + 4 * N * k
-    ws = (p + 12 * N + 8 * N * k + 15) // 16 * 16
-    args = (ctypes.byref(io), ws, need)
+    io.logprob, io.entropy, io.rank, io.top_tokens, io.top_logprobs = [t.data_ptr() for t in out]
+    args = (ctypes.byref(io), ws.data_ptr() if need else 0, need)
     f = mk_build.load().lxm_score
     if torch.cuda.current_device() == i:
         e = f(*args, torch._C._cuda_getCurrentRawStream(i))

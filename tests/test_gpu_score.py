@@ -168,3 +168,19 @@ def test_long_sums_of_equal_terms(cuda):
     ref, entropy = -s.log(), s.log() + n * c * torch.exp(-c) / s
     assert (r.logprob.double().cpu() - ref.repeat(64)).abs().max() <= 2.0 ** -18
     assert (r.entropy.double().cpu() - entropy.repeat(64)).abs().max() <= 2.0 ** -17
+
+
+@pytest.mark.parametrize("N,V", [(3, 30000), (1100, 70)])
+def test_results_are_tensors_of_their_own(cuda, N, V):
+    """Each result may be kept, saved, changed in place or weighed with something that learns, whatever becomes of the
+    others and of the call's workspace."""
+    print(f"[gpu-test] score results {N}x{V}", flush=True)
+    r = token_logprobs(torch.randn(N, V, device=cuda), torch.zeros(N, dtype=torch.int32, device=cuda), 5)
+    assert all(t._base is None and t.untyped_storage().nbytes() == t.numel() * t.element_size() for t in r)
+    w = torch.ones(N, device=cuda, requires_grad=True)
+    loss = (w * r.logprob).sum()
+    r.rank.add_(1), r.top_tokens.zero_()
+    loss.backward()
+    assert torch.equal(w.grad, r.logprob)
+    r.logprob.mul_(w)
+    assert r.logprob.requires_grad
