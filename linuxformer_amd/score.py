@@ -13,8 +13,10 @@ import operator
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import mk_build
+from .seqs import refuse_gradients
 
 TOP_MAX = 64  # alternatives at most (LXM_SCORE_TOP)
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -47,8 +49,8 @@ def token_logprobs(logits, tokens, top=0):
     i = logits.get_device()
     if tokens.get_device() != i:
         raise ValueError(f"token_logprobs: logits on {logits.device}, tokens on {tokens.device}")
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("no gradients are formed here: call under torch.no_grad()")
+    if logits.requires_grad or forward_ad._current_level >= 0:
+        refuse_gradients(logits)
     top = operator.index(top)  # (its value: a tensor's may change)
     key = (logits.shape, logits.stride(), logits.dtype, tokens.shape, tokens.stride(), tokens.dtype, top, i)
     call = _calls.get(key)

@@ -18,6 +18,7 @@ import ctypes
 from array import array
 
 import torch
+from torch.autograd import forward_ad
 
 from . import mk_build
 
@@ -146,12 +147,20 @@ def _launch(seqs, f, *args):
         raise RuntimeError(f"{f.__name__} failed: hipError {e}")
 
 
-def _elsewhere(seqs, *tensors):
-    """Why these tensors cannot be used with the sequences (the callers have seen that they cannot)."""
+def refuse_gradients(*tensors):
+    """What needs a gradient, backward or forward, while gradients are formed at all, is refused (None is skipped)."""
     for t in tensors:
-        if t.device != seqs.device:
-            return ValueError(f"a tensor on {t.device}, the sequences on {seqs.device}")
-    return RuntimeError("no gradients are formed here: call under torch.no_grad()")
+        if t is not None and (torch.is_grad_enabled() and t.requires_grad or
+                              forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None):
+            raise RuntimeError("no gradients are formed here: call under torch.no_grad(), without tangents")
+
+
+def _refuse(seqs, *tensors):
+    """Tensors elsewhere than the sequences or with gradients to be formed (None is skipped)."""
+    for t in tensors:
+        if t is not None and t.device != seqs.device:
+            raise ValueError(f"a tensor on {t.device}, the sequences on {seqs.device}")
+    refuse_gradients(*tensors)
 
 
 _calls = {}  # what calls of given shapes, strides and types pass on, their checks done
@@ -194,9 +203,10 @@ def short_conv(x, w, window, seqs, out=None):
     must not overlap x) those rows are left as they were."""
     i = seqs.index
     if x.get_device() != i or w.get_device() != i or window.get_device() != i or \
-            (out is not None and out.get_device() != i) or \
+            (out is not None and (out.get_device() != i or out.requires_grad)) or \
+            forward_ad._current_level >= 0 or \
             (torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or window.requires_grad)):
-        raise _elsewhere(seqs, x, w, window, *([] if out is None else [out]))
+        _refuse(seqs, x, w, window, out)
     if out is not None:
         _check_out(out, x, "x")
     y = _new_out(x, seqs) if out is None else out
@@ -248,10 +258,11 @@ def gated_delta(q, k, v, g, beta, state, seqs, scale=None, unit=True, out=None):
     i = seqs.index
     if q.get_device() != i or k.get_device() != i or v.get_device() != i or g.get_device() != i or \
             beta.get_device() != i or state.get_device() != i or \
-            (out is not None and out.get_device() != i) or (torch.is_grad_enabled() and (
+            (out is not None and (out.get_device() != i or out.requires_grad)) or \
+            forward_ad._current_level >= 0 or (torch.is_grad_enabled() and (
                 q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or
                 beta.requires_grad or state.requires_grad)):
-        raise _elsewhere(seqs, q, k, v, g, beta, state, *([] if out is None else [out]))
+        _refuse(seqs, q, k, v, g, beta, state, out)
     if out is not None:
         _check_out(out, v, "v")
     o = _new_out(v, seqs) if out is None else out

@@ -25,3 +25,10 @@ def test_token_logprobs_refuses(logits, tokens, top):
 def test_token_logprobs_refuses_gradients():
     with torch.enable_grad(), pytest.raises(RuntimeError, match="gradients"):
         token_logprobs(torch.zeros(2, 8, requires_grad=True), torch.zeros(2, dtype=torch.int64))
+
+
+def test_token_logprobs_refuses_tangents():
+    with torch.autograd.forward_ad.dual_level():
+        x = torch.autograd.forward_ad.make_dual(torch.zeros(2, 8), torch.ones(2, 8))
+        with pytest.raises(RuntimeError, match="gradients"):
+            token_logprobs(x, torch.zeros(2, dtype=torch.int64))

@@ -96,3 +96,38 @@ def test_scale_and_unit_are_read_at_each_call(monkeypatch):
     scale.fill_(0.25), unit.fill_(False)
     gated_delta(*a, plan, scale=scale, unit=unit)
     assert seen == [(0.5, 1), (0.25, 0)]
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "g", "beta", "state"])
+def test_gated_delta_refuses_tangents(name):
+    a = dict(_delta(), seqs=Sequences([5], device="cpu"))
+    with torch.autograd.forward_ad.dual_level():
+        a[name] = torch.autograd.forward_ad.make_dual(a[name], torch.ones_like(a[name]))
+        with pytest.raises(RuntimeError, match="gradients"):
+            gated_delta(**a)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="gradients"):  # (tangents are formed there, too)
+            gated_delta(**a)
+        with torch.inference_mode(), pytest.raises(ValueError, match="run on a GPU"):  # (not here)
+            gated_delta(**a)
+
+
+@pytest.mark.parametrize("name", ["x", "w", "window"])
+def test_short_conv_refuses_tangents(name):
+    a = dict(x=torch.zeros(5, 8), w=torch.zeros(8, 4), window=torch.zeros(2, 8, 4), seqs=Sequences([2, 3], device="cpu"))
+    with torch.autograd.forward_ad.dual_level():
+        a[name] = torch.autograd.forward_ad.make_dual(a[name], torch.ones_like(a[name]))
+        with pytest.raises(RuntimeError, match="gradients"):
+            short_conv(**a)
+
+
+def test_an_out_that_needs_a_gradient_is_refused():
+    a = dict(_delta(), seqs=Sequences([5], device="cpu"), out=torch.zeros(5, 4, 32, dtype=torch.bfloat16, requires_grad=True))
+    c = dict(x=torch.zeros(5, 8), w=torch.zeros(8, 4), window=torch.zeros(2, 8, 4), seqs=Sequences([2, 3], device="cpu"),
+             out=torch.zeros(5, 8, requires_grad=True))
+    with torch.enable_grad():
+        with pytest.raises(RuntimeError, match="gradients"):
+            gated_delta(**a)
+        with pytest.raises(RuntimeError, match="gradients"):
+            short_conv(**c)
+    with torch.no_grad(), pytest.raises(ValueError, match="run on a GPU"):
+        gated_delta(**a)
