@@ -19,6 +19,7 @@ from array import array
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import mk_build
 
@@ -163,6 +164,14 @@ def _refuse(seqs, *tensors):
     refuse_gradients(*tensors)
 
 
+def _written(*tensors):
+    """Tells autograd that the kernels change these in place: what saved one for its backward pass fails there instead
+    of taking the new values."""
+    for t in tensors:
+        if not t.is_inference():
+            increment_version(t)
+
+
 _calls = {}  # what calls of given shapes, strides and types pass on, their checks done
 
 
@@ -225,6 +234,7 @@ def short_conv(x, w, window, seqs, out=None):
     io = ConvIO.from_buffer_copy(io)
     io.x, io.w, io.window, io.y = x.data_ptr(), w.data_ptr(), window.data_ptr(), y.data_ptr()
     _launch(seqs, mk_build.load().lxm_short_conv, ctypes.byref(seqs.table), ctypes.byref(io))
+    _written(*((window,) if out is None else (window, out)))
     return y
 
 
@@ -297,6 +307,7 @@ def gated_delta(q, k, v, g, beta, state, seqs, scale=None, unit=True, out=None):
         n = max(least.value, min(n.value, WS_MAX))
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         _launch(seqs, lib.lxm_gd_chunks, ctypes.byref(seqs.table), ctypes.byref(io), ws.data_ptr(), n)
+    _written(*((state,) if out is None else (state, out)))
     return o
 
 

@@ -131,3 +131,28 @@ def test_an_out_that_needs_a_gradient_is_refused():
             short_conv(**c)
     with torch.no_grad(), pytest.raises(ValueError, match="run on a GPU"):
         gated_delta(**a)
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_autograd_sees_what_is_written(monkeypatch, inference):
+    """A cache or an out that something saved for its backward pass counts as changed (an inference tensor is never
+    saved, and has no count)."""
+    monkeypatch.setattr(seqs, "_launch", lambda *a: None)
+    monkeypatch.setattr(seqs.mk_build, "load", lambda: SimpleNamespace(lxm_gd_recurrent=None, lxm_short_conv=None))
+    plan = Sequences([1], device="cpu")
+    with torch.inference_mode(inference):
+        a = [torch.zeros(s) for s in ((1, 1, 64), (1, 1, 64), (1, 1, 16), (1, 1), (1, 1), (1, 1, 64, 16))]
+        c = [torch.zeros(s) for s in ((1, 8), (8, 4), (1, 8, 4))]
+        out, y = torch.zeros(1, 1, 16), torch.zeros(1, 8)
+    gated_delta(*a, plan, out=out), short_conv(*c, plan, out=y)
+    if inference:
+        return
+    assert [t._version for t in a + [out] + c + [y]] == [0, 0, 0, 0, 0, 1, 1, 0, 0, 1, 1]
+    gated_delta(*a, plan), short_conv(*c, plan)
+    assert [t._version for t in a + [out] + c + [y]] == [0, 0, 0, 0, 0, 2, 1, 0, 0, 2, 1]
+    w = torch.ones(1, 1, 64, 16, requires_grad=True)
+    with torch.enable_grad():
+        loss = (w * a[5]).sum()
+    gated_delta(*a, plan)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
