@@ -72,7 +72,6 @@ __device__ __forceinline__ int token_of(double key) { return (int)(0x7fffffffu -
 struct Lds {
   __attribute__((aligned(16))) double list[kWaves][kList + 8];
   __attribute__((aligned(16))) double all[kThreads + 8];  // the waves' best, and the workgroup's
-  __attribute__((aligned(16))) double high[kWaves][64];
   int n[kWaves];
   float m[kWaves], s[kWaves], w[kWaves];
   int c[kWaves];
@@ -456,10 +455,10 @@ bool bad(const lxm_score_io* io) {
 // How many parts a row is split into: enough for 4 workgroups a CU, each of at least 4,096 elements (top 8, least of
 // 4,096 / 8,192 / 32,768: one row of 459,982 in 14.8 / 15.4 / 20.5 us, 61 of 31,999 in 15.2 / 15.7 / 25.1; 2 and 8
 // workgroups a CU: 600 rows of 248,320 94.7 and 91.4 against 89.2).
-constexpr int kLeast = 4096;
+constexpr int kLeast = 4096, kRows = 0xffffffffu / kThreads;
 int parts_of(const lxm_score_io* io) {
   const int64_t most = ((int64_t)io->V + kLeast - 1) / kLeast;
-  int64_t n = io->rows > 0 ? (1024 + io->rows - 1) / io->rows : 1;
+  int64_t n = io->rows > 0 ? ((int64_t)io->rows + 1023) / io->rows : 1;
   return (int)(n > most ? most : n < 1 ? 1 : n);
 }
 
@@ -468,16 +467,23 @@ int launch(const lxm_score_io* io, char* ws, hipStream_t st) {
   const int vec = TY == 2 ? 4 : 8, n = parts_of(io);
   const int64_t words = (int64_t)io->V / vec;
   const int per = (int)((words + n - 1) / n) + (words < n);  // (at least 1)
-  if ((int64_t)io->rows * n > 0x7fffffff) return hipErrorInvalidValue;
   Part* parts = (Part*)ws;
   double* lists = (double*)(ws + (int64_t)io->rows * n * sizeof(Part));
   // Blocks of 16 elements a lane for a part that is one block, of 32 for whole rows, whose loads they keep in flight
   // (2,048 rows of 248,320, top 8: 210 us, in blocks of 8 219).
-  if (n > 1) {
+  if (n > 1) {  // (rows x n <= 2,046)
     score_part<TY, 16><<<io->rows * n, kThreads, 0, st>>>(*io, n, per, parts, lists);
     score_join<TY><<<io->rows, kThreads, 0, st>>>(*io, n, parts, lists);
   } else {
-    score_part<TY, 32><<<io->rows, kThreads, 0, st>>>(*io, n, per, parts, lists);
+    lxm_score_io r = *io;
+    for (int left = io->rows; left > 0; left -= kRows) {  // (a launch's threads are counted in 32 bits)
+      score_part<TY, 32><<<left < kRows ? left : kRows, kThreads, 0, st>>>(r, n, per, parts, lists);
+      if (int e = hipGetLastError()) return e;
+      r.logits = (const char*)r.logits + kRows * r.stride * (TY == 2 ? 4 : 2);
+      r.tokens = (const char*)r.tokens + (int64_t)kRows * (r.wide ? 8 : 4);
+      r.logprob += kRows, r.entropy += kRows, r.rank += kRows;
+      r.top_tokens += (int64_t)kRows * r.top, r.top_logprobs += (int64_t)kRows * r.top;
+    }
   }
   return hipGetLastError();
 }

@@ -940,6 +940,9 @@ __global__ __launch_bounds__(512, TY == LXM_BF16 && K <= 128 ? 4 : 2) void gd_ru
 }
 
 // ---- host ---------------------------------------------------------------------------------------------
+// workgroups of a launch at most: its threads are counted in 32 bits
+constexpr int64_t most(int threads) { return 0xffffffffll / threads; }
+
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 bool bad_table(const lxm_seq_table* s) {
@@ -966,35 +969,37 @@ int recurrent(const lxm_seq_table* s, const lxm_gd_io* io, hipStream_t st) {
   // in 16; one token of 64 sequences 39.5 in 128, 64.9 in 16.
   int cb = 128;
   while (cb > 16 && (io->V % cb || heads * (io->V / cb) < 512)) cb /= 2;
-  const int64_t grid = heads * (io->V / cb);
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  if (cb == 128) gd_recurrent<TY, K, 128><<<(int)grid, 256, 0, st>>>(*s, *io);
-  else if (cb == 64) gd_recurrent<TY, K, 64><<<(int)grid, 256, 0, st>>>(*s, *io);
-  else if (cb == 32) gd_recurrent<TY, K, 32><<<(int)grid, 256, 0, st>>>(*s, *io);
-  else gd_recurrent<TY, K, 16><<<(int)grid, 256, 0, st>>>(*s, *io);
-  return hipGetLastError();
+  const int each = io->nk * io->r * (io->V / cb), step = (int)(most(256) / each);  // (each <= 2^20: bad_io)
+  lxm_seq_table t = *s;
+  for (int left = s->n_seqs; left > 0; left -= step, t.seqs += 4 * (int64_t)step) {
+    const int grid = (left < step ? left : step) * each;
+    if (cb == 128) gd_recurrent<TY, K, 128><<<grid, 256, 0, st>>>(t, *io);
+    else if (cb == 64) gd_recurrent<TY, K, 64><<<grid, 256, 0, st>>>(t, *io);
+    else if (cb == 32) gd_recurrent<TY, K, 32><<<grid, 256, 0, st>>>(t, *io);
+    else gd_recurrent<TY, K, 16><<<grid, 256, 0, st>>>(t, *io);
+    if (int e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
 }
 
 constexpr int64_t kTwo = 600;
 
 template <int TY, int K>
 int chunks(const lxm_seq_table* s, const lxm_gd_io* io, char* ws, int64_t ws_bytes, hipStream_t st) {
-  const int nv = io->nk * io->r, per = (nv + 7) / 8;
+  const int nv = io->nk * io->r, per = (nv + 7) / 8, preps = io->nk * ((io->r + 3) / 4);
   const int64_t carry = 2 * (int64_t)nv * K * io->V * 4, each = (int64_t)io->nk * kKeyWs<TY, K> + (int64_t)nv * kHeadWs;
   if (ws_bytes < carry + each) return hipErrorInvalidValue;
   int64_t group = (ws_bytes - carry) / each;
   if (group > s->n_chunks) group = s->n_chunks;
-  if (group * nv > 0x7fffffff) group = 0x7fffffff / nv;
+  if (group > most(256) / preps) group = most(256) / preps;
   // Two column blocks a workgroup share its left operands, one has the shorter chain: two where, over the time of the
   // longest sequence's chain, that many workgroups of one block would be at work on average. 128 x 128, one against
   // two: a prompt of 2,048 in 32 heads (256 at work) 68 us against 84, in 64 heads (512) 95 and 95, in 128
   // (1,024) 196 and 166; 24 ragged prompts (1,300) 117 and 97, in fp32 297 and 232; fp32 with 256
   // x 128, where two spill 31 registers, 289 and 248 still.
-  const int64_t one = (int64_t)s->n_seqs * 8 * per * (io->V / 16);
   const int64_t chain = (s->max_len + LXM_SEQ_CHUNK - 1) / LXM_SEQ_CHUNK;
   const bool two = io->V % 32 == 0 && s->n_chunks * (int64_t)nv * (io->V / 16) >= kTwo * chain;
-  const int64_t grid = two ? one / 2 : one;
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  const int runs = 8 * per * (io->V / (two ? 32 : 16)), step = (int)(most(512) / runs);  // (of a sequence; runs <= 2^20)
   const int mats = (io->r < 4 ? io->r : 4) * kMat;
   const int lds = (int)sizeof(PrepLds) + (mats > kStage<TY, K> ? mats : kStage<TY, K>);
   // (on every call: the attribute is the current device's)
@@ -1003,10 +1008,15 @@ int chunks(const lxm_seq_table* s, const lxm_gd_io* io, char* ws, int64_t ws_byt
   float* carries[2] = {(float*)ws, (float*)(ws + carry / 2)};
   for (int64_t c0 = 0, turn = 0; c0 < s->n_chunks; c0 += group, turn = !turn) {
     const int n = (int)(s->n_chunks - c0 < group ? s->n_chunks - c0 : group);
-    gd_prep<TY, K><<<n * io->nk * ((io->r + 3) / 4), 256, lds, st>>>(*s, *io, ws + carry, (int)c0);
-    if (two) gd_run<TY, K, 2><<<(int)grid, 512, 0, st>>>(*s, *io, ws + carry, (int)c0, n, carries[turn], carries[!turn]);
-    else gd_run<TY, K, 1><<<(int)grid, 512, 0, st>>>(*s, *io, ws + carry, (int)c0, n, carries[turn], carries[!turn]);
+    gd_prep<TY, K><<<n * preps, 256, lds, st>>>(*s, *io, ws + carry, (int)c0);
     if (int e = hipGetLastError()) return e;
+    lxm_seq_table t = *s;
+    for (int left = s->n_seqs; left > 0; left -= step, t.seqs += 4 * (int64_t)step) {
+      const int grid = (left < step ? left : step) * runs;
+      if (two) gd_run<TY, K, 2><<<grid, 512, 0, st>>>(t, *io, ws + carry, (int)c0, n, carries[turn], carries[!turn]);
+      else gd_run<TY, K, 1><<<grid, 512, 0, st>>>(t, *io, ws + carry, (int)c0, n, carries[turn], carries[!turn]);
+      if (int e = hipGetLastError()) return e;
+    }
   }
   return hipSuccess;
 }
@@ -1016,12 +1026,17 @@ int conv(const lxm_seq_table* s, const lxm_conv_io* io, hipStream_t st) {
   const int vec = kVec<TY>, runs = (min(s->max_len, LXM_SEQ_CHUNK) + kRun - 1) / kRun;
   const bool wide = io->C % vec == 0 && io->x_ts % vec == 0 && io->y_ts % vec == 0 && io->w_ss % vec == 0 && aligned(io->x) &&
                     aligned(io->y) && aligned(io->w) && aligned(io->window);
-  const int cblocks = (io->C + 256 * (wide ? vec : 1) - 1) / (256 * (wide ? vec : 1));
-  const int64_t grid = (int64_t)cblocks * runs * s->n_chunks;
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  if (wide) short_conv<TY, kVec<TY>><<<(int)grid, 256, 0, st>>>(*s, *io, runs, cblocks);
-  else short_conv<TY, 1><<<(int)grid, 256, 0, st>>>(*s, *io, runs, cblocks);
-  return hipGetLastError();
+  const int64_t cols = 256 * (wide ? vec : 1), cblocks = (io->C + cols - 1) / cols, each = cblocks * runs;
+  if (each > most(256) || cblocks * cols > 0x7fffffff) return hipErrorInvalidValue;
+  const int step = (int)(most(256) / each);
+  lxm_seq_table t = *s;
+  for (int left = s->n_chunks; left > 0; left -= step, t.chunks += 4 * (int64_t)step) {
+    const int grid = (int)((left < step ? left : step) * each);
+    if (wide) short_conv<TY, kVec<TY>><<<grid, 256, 0, st>>>(t, *io, runs, (int)cblocks);
+    else short_conv<TY, 1><<<grid, 256, 0, st>>>(t, *io, runs, (int)cblocks);
+    if (int e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
 }
 
 #define BY_TYPE(ty, f, ...)                                  \

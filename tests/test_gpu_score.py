@@ -184,3 +184,21 @@ def test_results_are_tensors_of_their_own(cuda, N, V):
     assert torch.equal(w.grad, r.logprob)
     r.logprob.mul_(w)
     assert r.logprob.requires_grad
+
+
+def test_more_rows_than_a_launch_holds(cuda):
+    """A launch's threads are counted in 32 bits: rows past 16,777,215 workgroups of 256 go in another."""
+    print("[gpu-test] score of many rows", flush=True)
+    N = 16_777_300
+    x, t = torch.randn(N, 2, device=cuda), torch.randint(0, 2, (N,), dtype=torch.int32, device=cuda)
+    r = token_logprobs(x, t, 1)
+    lp = torch.log_softmax(x.double(), 1)
+    ref = lp.gather(1, t[:, None].long())[:, 0]
+    best = x.max(1)
+    first = torch.where(x[:, 0] == x[:, 1], 0, best.indices)
+    assert ((r.logprob - ref).abs() <= 2.0 ** -17 * (1 + ref.abs())).all()
+    entropy = -(lp.exp() * lp).sum(1)
+    assert ((r.entropy - entropy).abs() <= 2.0 ** -16 * (1 + entropy)).all()
+    assert torch.equal(r.top_tokens[:, 0].long(), first) and torch.equal(r.rank, (t != first).int())
+    assert torch.equal(r.top_logprobs[:, 0].isfinite(), torch.ones_like(first, dtype=torch.bool))
+    assert torch.equal(torch.where(t == first, r.top_logprobs[:, 0], r.logprob), r.logprob)
