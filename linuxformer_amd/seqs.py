@@ -232,7 +232,8 @@ def short_conv(x, w, window, seqs, out=None):
         y[:seqs.n_tokens] = z[:seqs.n_tokens]
         return y
     io = ConvIO.from_buffer_copy(io)
-    io.x, io.w, io.window, io.y = x.data_ptr(), w.data_ptr(), window.data_ptr(), y.data_ptr()
+    io.x, io.w, io.y = x.data_ptr(), w.data_ptr(), y.data_ptr()
+    io.window = window.data_ptr() or io.y  # (a cache of no slots has no address, and none is read)
     _launch(seqs, mk_build.load().lxm_short_conv, ctypes.byref(seqs.table), ctypes.byref(io))
     _written(*((window,) if out is None else (window, out)))
     return y
@@ -296,6 +297,7 @@ def gated_delta(q, k, v, g, beta, state, seqs, scale=None, unit=True, out=None):
         return o
     io = GdIO.from_buffer_copy(io)
     io.q, io.k, io.v, io.g, io.beta, io.state, io.o = p
+    io.state = p[5] or p[6]  # (a cache of no slots has no address, and none is read)
     lib = mk_build.load()
     if seqs.max_len <= (RECURRENT_MAX if seqs.n_seqs * v.shape[1] < MANY_HEADS else
                         RECURRENT_MAX_MANY[v.dtype]):
