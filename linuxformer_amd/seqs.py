@@ -192,8 +192,15 @@ def _fits(seqs, rows, slots):
 def _check_out(out, like, what):
     if out.shape != like.shape or out.dtype != like.dtype:
         raise ValueError(f"out: {what} as the input's, {tuple(like.shape)} {like.dtype}")
-    if any(out.stride(d) == 0 and out.shape[d] > 1 for d in range(out.dim())):
-        raise ValueError("out: elements that share memory")
+
+
+def _apart(out):
+    """Refuses a tensor two of whose elements may share memory: a dimension's step is past all that lies within it."""
+    end = 0
+    for step, n in sorted((out.stride(d), out.shape[d]) for d in range(out.dim()) if out.shape[d] > 1):
+        if step <= end:
+            raise ValueError("out: elements that share memory")
+        end += (n - 1) * step
 
 
 def _new_out(like, seqs):
@@ -247,6 +254,7 @@ def _conv_io(x, w, window, y):
         raise ValueError("short_conv: x (N, C), w (C, 4), window (slots, C, 4)")
     if not _dense(window, 1) or (window.shape[0] > 1 and window.stride(0) < 4 * C):
         raise ValueError("short_conv: a slot's window is dense, and the slots lie apart")
+    _apart(y)
     if not (_dense(x, 1) and _dense(w, 0) and _dense(y, 1)):
         return False
     return ConvIO(0, 0, 0, 0, _step(x, 0), _step(window, 0), _step(y, 0), C, TYPES[x.dtype])
@@ -333,6 +341,7 @@ def _delta_io(q, k, v, g, beta, state, o, scale, unit):
     if not _dense(state, 1) or _step(state, 0) % 4 or \
             (state.shape[0] > 1 and state.stride(0) < nv * K * V):
         raise ValueError("gated_delta: a slot's state is dense and 16-byte aligned, and the slots lie apart")
+    _apart(o)
     if not (_aligned(q) and _aligned(k) and _aligned(v) and _aligned(o)):
         return False
     return GdIO(0, 0, 0, 0, 0, 0, 0, _step(q, 0), _step(q, 1), _step(k, 0), _step(k, 1), _step(v, 0),

@@ -156,3 +156,20 @@ def test_autograd_sees_what_is_written(monkeypatch, inference):
     gated_delta(*a, plan)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_an_out_whose_rows_overlap_is_refused():
+    """Rows that reach into the next, in any order of the dimensions; views of a larger buffer do not."""
+    plan, buf = Sequences([5], device="cpu"), torch.zeros(5, 6, 48)
+    a = _delta(dt=torch.float32)
+    for shape, strides in (((5, 4, 32), (64, 16, 1)), ((5, 4, 32), (16, 64, 1)), ((5, 4, 32), (128, 1, 1))):
+        with pytest.raises(ValueError, match="share memory"):
+            gated_delta(**a, seqs=plan, out=torch.as_strided(buf, shape, strides))
+    for out in (buf[:, 1:5, 16:], buf.view(6, 5, 48).transpose(0, 1)[:, 2:, :32]):
+        with pytest.raises(ValueError, match="run on a GPU"):
+            gated_delta(**a, seqs=plan, out=out)
+    c = dict(x=torch.zeros(5, 8), w=torch.zeros(8, 4), window=torch.zeros(1, 8, 4), seqs=plan)
+    with pytest.raises(ValueError, match="share memory"):
+        short_conv(**c, out=torch.as_strided(buf, (5, 8), (4, 1)))
+    with pytest.raises(ValueError, match="run on a GPU"):
+        short_conv(**c, out=buf[:, 0, :8])
