@@ -205,7 +205,7 @@ def _apart(out):
 
 def _new_out(like, seqs):
     out = like.new_empty(like.shape)
-    if like.shape[0] > seqs.n_tokens:
+    if like.dim() and like.shape[0] > seqs.n_tokens:
         out[seqs.n_tokens:].zero_()
     return out
 

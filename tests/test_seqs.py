@@ -173,3 +173,11 @@ def test_an_out_whose_rows_overlap_is_refused():
         short_conv(**c, out=torch.as_strided(buf, (5, 8), (4, 1)))
     with pytest.raises(ValueError, match="run on a GPU"):
         short_conv(**c, out=buf[:, 0, :8])
+
+
+def test_a_tensor_of_no_dimensions_is_refused():
+    a = dict(_delta(), seqs=Sequences([5], device="cpu"), v=torch.zeros((), dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        gated_delta(**a)
+    with pytest.raises(ValueError):
+        short_conv(torch.zeros(()), torch.zeros(8, 4), torch.zeros(1, 8, 4), Sequences([5], device="cpu"))
