@@ -950,10 +950,13 @@ bool bad_table(const lxm_seq_table* s) {
          (s->n_seqs && (!s->seqs || !aligned(s->seqs))) || (s->n_chunks && (!s->chunks || !aligned(s->chunks)));
 }
 
+bool bad_shape(const lxm_gd_io* io) {
+  return !io || io->nk < 1 || io->r < 1 || (int64_t)io->nk * io->r > 65536 || (io->K != 64 && io->K != 128 && io->K != 256) || io->V < 16 ||
+         io->V > 256 || io->V % 16 || io->type < 0 || io->type > 2;
+}
+
 bool bad_io(const lxm_gd_io* io) {
-  if (!io || io->nk < 1 || io->r < 1 || (int64_t)io->nk * io->r > 65536 || (io->K != 64 && io->K != 128 && io->K != 256) || io->V < 16 ||
-      io->V > 256 || io->V % 16 || io->type < 0 || io->type > 2 || io->beta_type < 0 || io->beta_type > 2)
-    return true;
+  if (bad_shape(io) || io->beta_type < 0 || io->beta_type > 2) return true;
   const int64_t vec = io->type == LXM_FP32 ? 4 : 8;
   return !io->q || !io->k || !io->v || !io->g || !io->beta || !io->state || !io->o || !aligned(io->q) ||
          !aligned(io->k) || !aligned(io->v) || !aligned(io->state) || !aligned(io->o) || io->q_ts % vec || io->q_hs % vec ||
@@ -1075,7 +1078,7 @@ extern "C" int lxm_gd_recurrent(const lxm_seq_table* s, const lxm_gd_io* io, voi
 }
 
 extern "C" int lxm_gd_ws(const lxm_gd_io* io, int32_t n_chunks, int64_t* bytes) {
-  if (!io || !bytes || n_chunks < 1) return hipErrorInvalidValue;
+  if (bad_shape(io) || !bytes || n_chunks < 1) return hipErrorInvalidValue;
   *bytes = BY_TYPE(io->type, ws_of, io, n_chunks);
   return hipSuccess;
 }

@@ -1,5 +1,6 @@
 """The batch's plan and what the batch functions refuse, on the CPU (a refused call launches nothing)."""
 
+import ctypes
 from types import SimpleNamespace
 
 import pytest
@@ -181,3 +182,10 @@ def test_a_tensor_of_no_dimensions_is_refused():
         gated_delta(**a)
     with pytest.raises(ValueError):
         short_conv(torch.zeros(()), torch.zeros(8, 4), torch.zeros(1, 8, 4), Sequences([5], device="cpu"))
+
+
+@pytest.mark.parametrize("change", [dict(K=96), dict(V=24), dict(V=272), dict(nk=0), dict(r=-1), dict(nk=70000), dict(type=3), dict()])
+def test_workspace_of_what_is_not_allowed(native_lib, change):
+    n = ctypes.c_int64(-1)
+    e = native_lib.lxm_gd_ws(ctypes.byref(seqs.GdIO(**{**dict(nk=2, r=2, K=128, V=64, type=0), **change})), 3, ctypes.byref(n))
+    assert (e, n.value) == (1, -1) if change else e == 0 and n.value > 0
