@@ -744,18 +744,22 @@ struct Run {
       for (int e = 0; e < 3; e++) f[p][e] = from[p][e][lane];
     issued();
   }
-  // S <- decay S + sum_i k_i e_i^T; then (wk, wh: the next chunk's) what the next needs for it
+  // S <- decay S + sum_i k_i e_i^T, the sum by itself and then one fma: added to the state part by part it would round
+  // the state each time; then (wk, wh: the next chunk's) what the next needs for it
   __device__ void step_state() {
 #pragma unroll
     for (int n = 0; n < NC; n++) {
       u32x4 ef[2][3];
       operand(ef, m.e[n]);
-#pragma unroll
-      for (int t = 0; t < NT; t++) s[n][t] *= eg;
+      f32x4 a[NT] = {};
 #pragma unroll
       for (int p = 0; p < 2; p++)
 #pragma unroll
-        for (int t = 0; t < NT; t++) s[n][t] = product<NP, 3>(xf[t][p], ef[p], s[n][t]);
+        for (int t = 0; t < NT; t++) a[t] = product<NP, 3>(xf[t][p], ef[p], a[t]);
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[n][t][r] = fma(eg, s[n][t][r], a[t][r]);
     }
     put_state();
     load_x();
@@ -888,8 +892,8 @@ struct Run {
   }
 };
 
-// (Four waves a SIMD where the registers allow it, two workgroups a CU: 24 ragged prompts of bf16 118 us with 4
-// registers spilled, 139 with 136 registers and one workgroup.)
+// (Four waves a SIMD where the registers allow it, two workgroups a CU: 24 ragged prompts of bf16 118 us, 139 with
+// 136 registers and one workgroup.)
 template <int TY, int K, int NC>
 __global__ __launch_bounds__(512, TY == LXM_BF16 && K <= 128 ? 4 : 2) void gd_run(lxm_seq_table S, lxm_gd_io io, const char* ws, int c0, int n_chunks,
                                               const float* carry, float* carry_to) {
