@@ -989,7 +989,7 @@ int recurrent(const lxm_seq_table* s, const lxm_gd_io* io, hipStream_t st) {
   return hipSuccess;
 }
 
-constexpr int64_t kTwo = 600;
+constexpr int64_t kTwo = 350;
 
 template <int TY, int K>
 int chunks(const lxm_seq_table* s, const lxm_gd_io* io, char* ws, int64_t ws_bytes, hipStream_t st) {
@@ -1001,9 +1001,9 @@ int chunks(const lxm_seq_table* s, const lxm_gd_io* io, char* ws, int64_t ws_byt
   if (group > most(256) / preps) group = most(256) / preps;
   // Two column blocks a workgroup share its left operands, one has the shorter chain: two where, over the time of the
   // longest sequence's chain, that many workgroups of one block would be at work on average. 128 x 128, one against
-  // two: a prompt of 2,048 in 32 heads (256 at work) 68 us against 84, in 64 heads (512) 95 and 95, in 128
-  // (1,024) 196 and 166; 24 ragged prompts (1,300) 117 and 97, in fp32 297 and 232; fp32 with 256
-  // x 128, where two spill 31 registers, 289 and 248 still.
+  // two: a prompt of 2,048 in 32 heads (256 at work) 68 us against 92, in 40 (320) 94 and 95, in 48 (384) 107
+  // and 104, in 64 127 and 118, in 128 254 and 216, in fp32 48 heads 224 and 181; 24 ragged prompts (1,300) 144 and
+  // 119, in fp32 306 and 240; fp32 with 256 x 128, where two spill 12 registers, 225 and 192.
   const int64_t chain = (s->max_len + LXM_SEQ_CHUNK - 1) / LXM_SEQ_CHUNK;
   const bool two = io->V % 32 == 0 && s->n_chunks * (int64_t)nv * (io->V / 16) >= kTwo * chain;
   const int runs = 8 * per * (io->V / (two ? 32 : 16)), step = (int)(most(512) / runs);  // (of a sequence; runs <= 2^20)
