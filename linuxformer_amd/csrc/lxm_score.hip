@@ -18,9 +18,9 @@
 // The rank: a token's own logit is compared with every element, from the float below it for lower tokens (equals count
 // there); where a block's maximum is below it nothing is.
 //
-// Bytes bound many rows: 2,048 rows of 248,320 bf16 logits, top 8, 214 us, 4.75 TB/s (179 with no alternatives; a list
+// Bytes bound many rows: 2,048 rows of 248,320 bf16 logits, top 8, 212 us, 4.8 TB/s (193 with no alternatives; a list
 // for the workgroup, a barrier a block, took 518). Few rows are split over parts (a workgroup each), joined by a
-// second kernel, and bound by the two kernels' latency: one row of 459,982, 7.8 and 6.8 us.
+// second kernel, and bound by the two kernels' latency: one row of 459,982, 7.9 and 7.1 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -231,7 +231,7 @@ struct Part {
 // One workgroup per (row, part). Between the row's first and last 16-byte boundary a part is whole words, dealt to the
 // waves 64 at a time, kEach elements a lane of a block; what the row has before and after (less than a word each) is
 // a block of one element a lane, before the first and after the last of the row. (Waves a SIMD: 2,048 bf16 rows of
-// 248,320 in 210 us with 5, 216 with 4; fp32 would spill 32 registers with 5, 1,200 rows of 150,001 in 223 us for 164.)
+// 248,320 in 212 us with 5, 215 with 4; fp32 would spill 32 registers with 5, 1,200 rows of 150,001 in 223 us for 164.)
 template <int TY, int kEach>
 __global__ __launch_bounds__(kThreads, TY == 2 ? 4 : 5) void score_part(lxm_score_io io, int n_parts, int words_per_part, Part* parts, double* lists) {
   typedef typename Elem<TY>::T T;

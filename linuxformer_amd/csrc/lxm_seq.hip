@@ -340,7 +340,7 @@ __global__ __launch_bounds__(256) void gd_recurrent(lxm_seq_table S, lxm_gd_io i
 // products. One such product of bf16 by float32 takes 3 instructions of 16 cycles per 32 k where the float32
 // instruction takes 8 of 32.
 //
-// 2,048 positions of 32 heads, bf16, 128 x 128: 60 to 68 us (gd_prep 17, gd_run 51), where the fp32 matrix
+// 2,048 positions of 32 heads, bf16, 128 x 128: 66 us (gd_prep 17, gd_run 56), where the fp32 matrix
 // instructions and a workspace of 75 KB a (head, chunk) take 234 for the same sums of float32 inputs.
 template <int TY>
 constexpr int kParts = TY == LXM_BF16 ? 1 : TY == LXM_FP16 ? 2 : 3;
@@ -492,7 +492,7 @@ __device__ __forceinline__ void invert(float* l, int lane) {
 // row's 8 elements of an operand), then T and A of each of the value heads from them. Decays are summed in
 // float64: behind a forgotten state (clamped to -1e5) the differences keep their digits.
 // Few chunks are bound by one workgroup's latency (17 us for 512, all at once on the card), many by the
-// workspace's bytes: 108 chunks of 16 key heads write 190 MB and read 67 in 51 us, 5 TB/s.
+// workspace's bytes: 98 chunks of 16 key heads write 191 MB and read 61 in 51 us, 4.9 TB/s.
 template <int TY, int K>
 __global__ __launch_bounds__(256) void gd_prep(lxm_seq_table S, lxm_gd_io io, char* ws, int c0) {
   typedef typename Elem<TY>::T T;
@@ -673,9 +673,9 @@ __global__ __launch_bounds__(256) void gd_prep(lxm_seq_table S, lxm_gd_io io, ch
 // D) cross the waves through LDS as parts. Waves 0 to 3 have a row tile of R and of D, which is the chain; waves
 // 4 to 7 one of the output, a step behind (S^T q while D is formed, A D in the next chunk's first step); all of
 // them their tiles of the state. What a chunk reads from memory is requested a chunk ahead, each register
-// again as soon as it has been used: nothing in the chain waits for memory. A chunk takes 1.5 us (3,250 cycles, of
-// which the MFMAs are 800 a SIMD): the parts' way through LDS (170 KB read), the operands' through the CU's vector
-// memory path (84 KB) and the barriers between them. In fp32 matrix instructions it took 5.6.
+// again as soon as it has been used: nothing in the chain waits for memory. A chunk takes 1.7 us (3,500 cycles, of
+// which the MFMAs are 1,090 a SIMD): the parts' way through LDS (192 KB read), the operands' through the CU's vector
+// memory path (90 KB) and the barriers between them. In fp32 matrix instructions it took 5.6.
 template <int TY, int K, int NC>
 struct Run {
   typedef typename Elem<TY>::T T;
@@ -788,7 +788,7 @@ struct Run {
     T v[NC][4];
     const int64_t ts = io.v_ts;
     const int row = w * 16 + 4 * g;
-    __builtin_amdgcn_s_setprio(2);  // (the chain's waves before the output's: prompt of 2,048 71.4 -> 68.2 us)
+    __builtin_amdgcn_s_setprio(2);  // (the chain's waves before the output's: prompt of 16,384 553.8 -> 551.7 us)
     vp += (t0 + row) * ts;
     auto load_v = [&] {
       if (t0 + LXM_SEQ_CHUNK <= end) {

@@ -27,12 +27,12 @@ CHUNK = 64              # positions per chunk (LXM_SEQ_CHUNK)
 # The longest sequences that go through the recurrence position by position: in calls of fewer than MANY_HEADS
 # (sequence, value head) pairs, and of more in bf16 and in fp16 and fp32 (whose chunks are split into more
 # products). 128 x 128, 32 heads, equal lengths, recurrence against chunks in us, of 1, 8 and 60 sequences:
-# 8 positions bf16 16 and 17, 20 and 31, 66 and 132; 12 bf16 22 and 18, fp32 21 and 20; 16 bf16 28 and 17, 32
-# and 31, 106 and 137; 24 bf16 40 and 18, 45 and 31, 148 and 146, fp16 41 and 19, 45 and 44, 149 and 245,
-# fp32 39 and 21, 46 and 47, 140 and 332; 32 fp32 50 and 21, 61 and 48, 181 and 337.
+# 8 positions bf16 16 and 18, 20 and 33, 66 and 143; 12 bf16 22 and 18, fp32 21 and 21; 16 bf16 28 and 18, 32
+# and 32, 106 and 146; 24 bf16 40 and 18, 45 and 33, 148 and 155, fp16 41 and 19, 45 and 45, 149 and 253,
+# fp32 39 and 21, 45 and 49, 140 and 341; 32 fp32 50 and 21, 60 and 49, 181 and 345.
 RECURRENT_MAX, MANY_HEADS = 8, 256
 RECURRENT_MAX_MANY = {torch.bfloat16: 16, torch.float16: 24, torch.float32: 24}
-WS_MAX = 192 << 20      # a call's workspace at most; more chunks go in groups
+WS_MAX = 192 << 20      # a call's workspace, unless one chunk needs more; more chunks go in groups
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 _P, _L, _I = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
@@ -59,7 +59,7 @@ class Sequences:
     """The sequences of a batch: their lengths (>= 0) and the slots of the caches they read and leave their
     state in. Slots of one batch are distinct; slot -1 (any number of them) starts from zeros and keeps
     nothing: padding, or a sequence that ends with the call. Default: slots 0, 1, 2, ... Lengths and slots are
-    host integers, checked here; the tables go to the device once. A graph that captured a call reads the
+    host integers, checked here; the tables go to the device once, by a copy that waits. A graph that captured a call reads the
     tables at every replay: the plan is to live as long."""
 
     def __init__(self, lengths, slots=None, device="cuda"):
@@ -272,8 +272,9 @@ def gated_delta(q, k, v, g, beta, state, seqs, scale=None, unit=True, out=None):
 
     Products and sums are float32's. Batches whose longest sequence has more than 8 positions (in large
     batches 16 in bfloat16, 24 in the others) go in chunks of 64 on the matrix cores, with a workspace of up
-    to WS_MAX bytes for the call; there, as in every chunked form, a NaN or infinity reaches the other
-    positions of its chunk. A view whose rows are not 16-byte aligned is copied first."""
+    to WS_MAX bytes for the call (or what two states of all heads and one chunk take: lxm_gd_ws); there, as in
+    every chunked form, a NaN or infinity reaches the other positions of its chunk. A view whose rows are not
+    16-byte aligned is copied first."""
     i = seqs.index
     if q.get_device() != i or k.get_device() != i or v.get_device() != i or g.get_device() != i or \
             beta.get_device() != i or state.get_device() != i or \
