@@ -59,8 +59,8 @@ class Sequences:
     """The sequences of a batch: their lengths (>= 0) and the slots of the caches they read and leave their
     state in. Slots of one batch are distinct; slot -1 (any number of them) starts from zeros and keeps
     nothing: padding, or a sequence that ends with the call. Default: slots 0, 1, 2, ... Lengths and slots are
-    host integers, checked here; the tables go to the device once, by a copy that waits. A graph that captured a call reads the
-    tables at every replay: the plan is to live as long."""
+    host integers, checked here; the tables go to the device once, by a copy that waits. A graph that captured
+    a call reads the tables at every replay: the plan is to live as long."""
 
     def __init__(self, lengths, slots=None, device="cuda"):
         lens = [int(n) for n in lengths]
@@ -270,11 +270,11 @@ def gated_delta(q, k, v, g, beta, state, seqs, scale=None, unit=True, out=None):
     by sqrt(sum of squares + 1e-6) first; scale: K ** -0.5 unless given. Returns o (N, nv, V), v's type; rows
     past the last sequence as in short_conv; out must not overlap the inputs.
 
-    Products and sums are float32's. Batches whose longest sequence has more than 8 positions (in large
-    batches 16 in bfloat16, 24 in the others) go in chunks of 64 on the matrix cores, with a workspace of up
-    to WS_MAX bytes for the call (or what two states of all heads and one chunk take: lxm_gd_ws); there, as in
-    every chunked form, a NaN or infinity reaches the other positions of its chunk. A view whose rows are not
-    16-byte aligned is copied first."""
+    Products and sums are float32's (in chunks, of numbers below 2^-110 only the leading digits count). Batches
+    whose longest sequence has more than 8 positions (in large batches 16 in bfloat16, 24 in the others) go in
+    chunks of 64 on the matrix cores, with a workspace of up to WS_MAX bytes for the call (or what two states of
+    all heads and one chunk take: lxm_gd_ws); there, as in every chunked form, a NaN or infinity reaches the
+    other positions of its chunk. A view whose rows are not 16-byte aligned is copied first."""
     i = seqs.index
     if q.get_device() != i or k.get_device() != i or v.get_device() != i or g.get_device() != i or \
             beta.get_device() != i or state.get_device() != i or \
